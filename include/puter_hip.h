@@ -289,6 +289,45 @@ PUTER_API int puter_hip_kv_page_write_fp8(void *storage, const void *values, con
                                           int64_t storage_offset, const float *scales, int value_dtype,
                                           int32_t *status, void *stream);
 
+/* Extension (no reference method): RoPE of Q and K and the KVPageWrite of K and V in
+ * one pass.  Row r of query [rows, query_heads * head_dim], key and value [rows,
+ * kv_heads * head_dim] (rows of one buffer or of several: the strides are elements from
+ * row to row) stands at position config->start_position + positions[r].  Q is rotated
+ * into query_out [rows, query_heads * head_dim] (which may be query where query_stride
+ * is a row's length); K is rotated, and K and V are stored at page page_ids[r], slot
+ * offsets[r] of the pools [page_count, page_size, kv_heads, head_dim].  Angles as
+ * puter_hip_rope; every value is rounded once, to what it is stored in.  config NULL: no
+ * rotation (positions is not read); query_heads 0: no queries.  cache_dtype:
+ *   - dtype itself (F32, F16, BF16): key_params and value_params are not read;
+ *   - PUTER_F8E4M3: byte = E4M3(value / scale), key_params / value_params hold the
+ *     fp32 scale of each kv head (as puter_hip_kv_page_write_fp8);
+ *   - PUTER_I4: head_dim 64, 128 or 256 in groups of `group` = 32, 64 or 128 dims.  The
+ *     pools hold packed signed nibbles [page_count, page_size, kv_heads, head_dim / 2],
+ *     key_params / value_params [page_count, page_size, kv_heads, head_dim / group]
+ *     pairs of f16 (scale, offset), written here; a value is scale * nibble + offset.
+ *     With lo and hi the least and greatest value of a group (kept to +-65504):
+ *     scale = f16((hi - lo) / 15), offset = f16((lo + hi) / 2 + scale / 2), nibble =
+ *     rint((x - offset) * (1 / scale)) in [-8, 7], 0 where scale is 0; a NaN makes its
+ *     group's scale and offset NaN.  Pools 16-byte aligned.
+ * Ids, slots, *status and several rows of one slot as puter_hip_kv_page_write; the query
+ * of a row that is not stored is still written.  head_dim: even, at most 1024. */
+PUTER_API int puter_hip_kv_page_append_rope(const puter_rope_config *config, const void *query, const void *key,
+                                            const void *value, const int32_t *positions, const int32_t *page_ids,
+                                            const int32_t *offsets, void *query_out, void *key_pages,
+                                            void *value_pages, void *key_params, void *value_params, int64_t rows,
+                                            int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                                            int64_t query_stride, int64_t key_stride, int64_t value_stride,
+                                            int64_t page_count, int64_t page_size, int64_t group, int dtype,
+                                            int cache_dtype, int32_t *status, void *stream);
+
+/* Extension: KVPageGather of a 4-bit pool as values: output [out_rows, kv_heads *
+ * head_dim] of dtype (F32, F16, BF16), row i from page page_table[i / page_size], slot
+ * i % page_size.  A bad id gives a zero row and *status, as puter_hip_kv_page_gather. */
+PUTER_API int puter_hip_kv_page_gather_int4(const void *pages, const void *params, const int32_t *page_table,
+                                            void *output, int64_t page_count, int64_t page_size, int64_t kv_heads,
+                                            int64_t head_dim, int64_t group, int64_t out_rows, int dtype,
+                                            int32_t *status, void *stream);
+
 /* ------------------------------------------------------------------------ */
 /* Attention: device/interface.go:91-110                                      */
 /* ------------------------------------------------------------------------ */
@@ -314,6 +353,24 @@ PUTER_API int puter_hip_multi_head_attention_batched(const puter_mha_config *con
                                            const void *key, const void *value, void *output,
                                            int64_t batch, int64_t seq_q, int64_t seq_k,
                                            int dtype, void *stream);
+
+/* Extension: MultiHeadAttention of `batch` sequences of different lengths in one call.
+ * Their rows stand back to back: sequence b's queries are rows query_offsets[b] ..
+ * query_offsets[b + 1] - 1 of query and output [total_q, H*D], its keys rows
+ * key_offsets[b] .. key_offsets[b + 1] - 1 of key and value [total_k, Hkv*D] (device
+ * arrays of batch + 1 int32; key_offsets NULL: query_offsets, total_k == total_q).
+ * Per sequence the masks of puter_hip_multi_head_attention with its own seqQ and seqK;
+ * score sums stay in f32 in every format.  A query that sees no key gives zeros, what a
+ * mask hides (NaN and infinities too) has no effect, and output rows before the first and
+ * from the last offset on are left as they were.  Offsets that are negative, fall or pass
+ * total_q / total_k store PUTER_ERR_INVALID into *status (NULL: not reported), and no
+ * access leaves the tensors.  F32, BF16, F16; head_dim at most 256 (the matrix cores take
+ * multiples of 8, of 4 in F32, in 16-byte aligned buffers). */
+PUTER_API int puter_hip_multi_head_attention_packed(const puter_mha_config *config, const void *query,
+                                                    const void *key, const void *value, void *output,
+                                                    const int32_t *query_offsets, const int32_t *key_offsets,
+                                                    int64_t batch, int64_t total_q, int64_t total_k, int dtype,
+                                                    int32_t *status, void *stream);
 
 /* FlashAttentionConfig, device/config.go:278-281. */
 typedef struct puter_flash_config {
@@ -362,6 +419,25 @@ PUTER_API int puter_hip_paged_decode_attention(const void *query, const void *ke
                                      int64_t max_context, const float *k_scale,
                                      const float *v_scale, int kv_dtype, void *output,
                                      void *workspace, size_t workspace_bytes, void *stream);
+
+/* Extension: attention over a paged cache in 4 bits (the pools and pairs that
+ * puter_hip_kv_page_append_rope writes with PUTER_I4).  query and output [batch,
+ * query_len, num_heads * head_dim] of dtype BF16 or F16; sequence b's cache holds
+ * context_lens[b] tokens (clamped to max_context), the last query_len of them its queries'
+ * own: query i sees the tokens up to context - query_len + i, and gives zeros where there
+ * is none.  page_table [batch, max_pages_per_seq]; a token whose page id is outside [0,
+ * num_pages) is masked, never read.  num_heads any multiple of kv_heads.  query, output,
+ * pools, pairs and workspace 16-byte aligned; workspace: caller-owned,
+ * puter_hip_paged_int4_workspace_bytes(...) bytes of any content, used by one call at a time. */
+PUTER_API size_t puter_hip_paged_int4_workspace_bytes(int64_t batch, int64_t query_len, int64_t num_heads,
+                                                      int64_t kv_heads, int64_t head_dim, int64_t max_context);
+PUTER_API int puter_hip_paged_int4_attention(const void *query, const void *key_pages, const void *value_pages,
+                                             const void *key_params, const void *value_params,
+                                             const int32_t *page_table, const int32_t *context_lens, int64_t batch,
+                                             int64_t query_len, int64_t max_pages_per_seq, int64_t page_size,
+                                             int64_t num_pages, int64_t num_heads, int64_t kv_heads,
+                                             int64_t head_dim, int64_t group, int64_t max_context, int dtype,
+                                             void *output, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ */
 /* Integer quantisation: Dequant / Dequant4 device/interface.go:196-199,       */

@@ -78,10 +78,15 @@ SIGNATURES = {
     "puter_hip_kv_page_write": ([vp] * 5 + [i64] * 5 + [i32, vp, vp], i32),
     "puter_hip_kv_page_gather": ([vp] * 3 + [i64] * 5 + [i32, vp, vp], i32),
     "puter_hip_kv_page_write_fp8": ([vp] * 4 + [i64] * 6 + [vp, i32, vp, vp], i32),
+    "puter_hip_kv_page_append_rope": ([C.POINTER(RopeConfig)] + [vp] * 11 + [i64] * 10 + [i32, i32, vp, vp],
+                                      i32),
+    "puter_hip_kv_page_gather_int4": ([vp] * 4 + [i64] * 6 + [i32, vp, vp], i32),
     "puter_hip_multi_head_attention": ([C.POINTER(MHAConfig), vp, vp, vp, vp, i64, i64, i32, vp],
                                        i32),
     "puter_hip_multi_head_attention_batched": ([C.POINTER(MHAConfig), vp, vp, vp, vp, i64, i64,
                                                 i64, i32, vp], i32),
+    "puter_hip_multi_head_attention_packed": ([C.POINTER(MHAConfig)] + [vp] * 6 + [i64] * 3 + [i32, vp, vp],
+                                              i32),
     "puter_hip_scaled_dot_product_attention": ([C.POINTER(FlashConfig), vp, vp, vp, vp, i64, i64,
                                                 i64, i64, i32, vp], i32),
     "puter_hip_flash_attention": ([C.POINTER(FlashConfig), vp, vp, vp, vp, i64, i64, i64, i64,
@@ -89,6 +94,8 @@ SIGNATURES = {
     "puter_hip_paged_decode_workspace_bytes": ([i64, i64, i64, i64], sz),
     "puter_hip_paged_decode_attention": ([vp] * 5 + [i64] * 8 + [vp, vp, i32, vp, vp, sz, vp],
                                          i32),
+    "puter_hip_paged_int4_workspace_bytes": ([i64] * 6, sz),
+    "puter_hip_paged_int4_attention": ([vp] * 7 + [i64] * 10 + [i32, vp, vp, sz, vp], i32),
     "puter_hip_dequant": ([vp, vp, i64, C.c_float, i32, i32, i32, vp], i32),
     "puter_hip_dequant4": ([vp, vp, i64, C.c_float, i32, i32, i32, vp], i32),
     "puter_hip_quant": ([vp, vp, i64, C.c_float, i32, i32, i32, vp], i32),

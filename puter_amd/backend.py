@@ -264,10 +264,14 @@ class Backend:
             _ptr(output), rows, lastDim, rowsPerBatch, modulationCols, set, format, self.stream()))
 
     # ---- RoPE family: device/interface.go:592-610 ----
+    @staticmethod
+    def _rope(config):
+        return _lib.RopeConfig(config.BaseFreq, config.StartPosition, config.Mode, config.Scaling,
+                               config.ScalingFactor, config.LowFreqFactor, config.HighFreqFactor,
+                               config.OriginalContext)
+
     def RoPE(self, config, input, output, seqLen, numHeads, headDim, format):
-        c = _lib.RopeConfig(config.BaseFreq, config.StartPosition, config.Mode, config.Scaling,
-                            config.ScalingFactor, config.LowFreqFactor, config.HighFreqFactor,
-                            config.OriginalContext)
+        c = self._rope(config)
         check(self.lib.puter_hip_rope(C.byref(c), _ptr(input), _ptr(output), seqLen, numHeads,
                                       headDim, format, self.stream()))
 
@@ -425,6 +429,30 @@ class Backend:
                                                    headDim, valueRows, storageOffset, _ptr(scales),
                                                    valueFormat, _ptr(self._status_word()), self.stream()))
 
+    def KVPageAppendRoPE(self, config, query, key, value, positions, pageIDs, offsets, queryOut,
+                         keyPages, valuePages, keyParams, valueParams, rows, queryHeads, kvHeads,
+                         headDim, queryStride, keyStride, valueStride, pageCount, pageSize, group,
+                         format, cacheFormat):
+        """Extension hook (no reference method): rotate the rows' Q and K at their own
+        positions, write Q out and store K and V in pages of the rows' format, F8E4M3
+        (keyParams / valueParams: the scale of each kv head) or I4 (the (scale, offset)
+        pairs of each group of dims, written).  config None: no rotation; queryHeads 0: no
+        queries.  Strides in elements."""
+        c = None if config is None else C.byref(self._rope(config))
+        check(self.lib.puter_hip_kv_page_append_rope(
+            c, _ptr(query), _ptr(key), _ptr(value), _ptr(positions), _ptr(pageIDs), _ptr(offsets),
+            _ptr(queryOut), _ptr(keyPages), _ptr(valuePages), _ptr(keyParams), _ptr(valueParams), rows,
+            queryHeads, kvHeads, headDim, queryStride, keyStride, valueStride, pageCount, pageSize,
+            group, format, cacheFormat, _ptr(self._status_word()), self.stream()))
+
+    def KVPageGatherInt4(self, pages, params, pageTable, output, pageCount, pageSize, kvHeads,
+                         headDim, group, outRows, format):
+        """Extension hook (no reference method): KVPageGather of a 4-bit pool, as values."""
+        check(self.lib.puter_hip_kv_page_gather_int4(_ptr(pages), _ptr(params), _ptr(pageTable),
+                                                     _ptr(output), pageCount, pageSize, kvHeads,
+                                                     headDim, group, outRows, format,
+                                                     _ptr(self._status_word()), self.stream()))
+
     # ---- Attention: device/interface.go:91-110 ----
     @staticmethod
     def _mha(config):
@@ -443,6 +471,16 @@ class Backend:
         check(self.lib.puter_hip_multi_head_attention_batched(C.byref(c), _ptr(query), _ptr(key),
                                                               _ptr(value), _ptr(output), batch,
                                                               seqQ, seqK, format, self.stream()))
+
+    def MultiHeadAttentionPacked(self, config, query, key, value, output, queryOffsets, keyOffsets,
+                                 batch, totalQ, totalK, format):
+        """Extension (no reference method): MultiHeadAttention of sequences of different
+        lengths whose rows stand back to back, parted by device offsets (batch + 1 int32;
+        keyOffsets None: the query offsets).  Bad offsets are reported by CheckStatus."""
+        c = self._mha(config)
+        check(self.lib.puter_hip_multi_head_attention_packed(
+            C.byref(c), _ptr(query), _ptr(key), _ptr(value), _ptr(output), _ptr(queryOffsets),
+            _ptr(keyOffsets), batch, totalQ, totalK, format, _ptr(self._status_word()), self.stream()))
 
     # device/interface.go:92-109 (single head; FlashAttention forwards to
     # ScaledDotProductAttention as device/cpu/attention/ops.go:21-31 does)
@@ -473,6 +511,22 @@ class Backend:
             batch, maxPagesPerSeq, pageSize, numPages, numHeads, kvHeads, headDim, maxContext,
             _ptr(kScale), _ptr(vScale), kvFormat, _ptr(output), _ptr(workspace), workspaceBytes,
             self.stream()))
+
+    def PagedInt4WorkspaceBytes(self, batch, queryLen, numHeads, kvHeads, headDim, maxContext):
+        return self.lib.puter_hip_paged_int4_workspace_bytes(batch, queryLen, numHeads, kvHeads,
+                                                             headDim, maxContext)
+
+    def PagedInt4Attention(self, query, keyPages, valuePages, keyParams, valueParams, pageTable,
+                           contextLens, batch, queryLen, maxPagesPerSeq, pageSize, numPages, numHeads,
+                           kvHeads, headDim, group, maxContext, format, output, workspace,
+                           workspaceBytes):
+        """Extension (no reference method): attention of one or a few query tokens per
+        sequence over a paged cache in 4 bits (KVPageAppendRoPE with I4)."""
+        check(self.lib.puter_hip_paged_int4_attention(
+            _ptr(query), _ptr(keyPages), _ptr(valuePages), _ptr(keyParams), _ptr(valueParams),
+            _ptr(pageTable), _ptr(contextLens), batch, queryLen, maxPagesPerSeq, pageSize, numPages,
+            numHeads, kvHeads, headDim, group, maxContext, format, _ptr(output), _ptr(workspace),
+            workspaceBytes, self.stream()))
 
     # ---- Dequant / Quant: device/interface.go:196-199, 580-582 ----
     def Dequant(self, dst, src, count, config, dstFormat, srcFormat):

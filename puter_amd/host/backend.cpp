@@ -17,6 +17,19 @@ std::string last_error(int status) {
     return m && *m ? std::string(m) : "puter_hip: status " + std::to_string(status);
 }
 
+puter_rope_config rope_config(const RoPEConfig &config) {
+    puter_rope_config c{};
+    c.base_freq = config.BaseFreq;
+    c.start_position = config.StartPosition;
+    c.mode = config.Mode;
+    c.scaling = config.Scaling;
+    c.scaling_factor = config.ScalingFactor;
+    c.low_freq_factor = config.LowFreqFactor;
+    c.high_freq_factor = config.HighFreqFactor;
+    c.original_context = config.OriginalContext;
+    return c;
+}
+
 puter_mha_config mha_config(const MultiHeadAttentionConfig &c) {
     puter_mha_config m{};
     m.num_heads = c.NumHeads;
@@ -234,15 +247,7 @@ void Backend::GatedResidualLayerNorm(const void *residual, const void *branch, c
 // ---- RoPE family -----------------------------------------------------------------------
 void Backend::RoPE(const RoPEConfig &config, const void *input, void *output, int64_t seqLen, int64_t numHeads,
                    int64_t headDim, DType format) {
-    puter_rope_config c{};
-    c.base_freq = config.BaseFreq;
-    c.start_position = config.StartPosition;
-    c.mode = config.Mode;
-    c.scaling = config.Scaling;
-    c.scaling_factor = config.ScalingFactor;
-    c.low_freq_factor = config.LowFreqFactor;
-    c.high_freq_factor = config.HighFreqFactor;
-    c.original_context = config.OriginalContext;
+    const puter_rope_config c = rope_config(config);
     Check(puter_hip_rope(&c, input, output, seqLen, numHeads, headDim, code(format), stream_));
 }
 
@@ -329,6 +334,30 @@ void Backend::KVPageWriteFP8(void *storage, const void *values, const void *page
                                       code(valueFormat), StatusWord(), stream_));
 }
 
+void Backend::KVPageAppendRoPE(const RoPEConfig *config, const void *query, const void *key, const void *value,
+                               const void *positions, const void *pageIDs, const void *offsets, void *queryOut,
+                               void *keyPages, void *valuePages, void *keyParams, void *valueParams, int64_t rows,
+                               int64_t queryHeads, int64_t kvHeads, int64_t headDim, int64_t queryStride,
+                               int64_t keyStride, int64_t valueStride, int64_t pageCount, int64_t pageSize,
+                               int64_t group, DType format, DType cacheFormat) {
+    const puter_rope_config c = config ? rope_config(*config) : puter_rope_config{};
+    Check(puter_hip_kv_page_append_rope(config ? &c : nullptr, query, key, value,
+                                        static_cast<const int32_t *>(positions),
+                                        static_cast<const int32_t *>(pageIDs),
+                                        static_cast<const int32_t *>(offsets), queryOut, keyPages, valuePages,
+                                        keyParams, valueParams, rows, queryHeads, kvHeads, headDim, queryStride,
+                                        keyStride, valueStride, pageCount, pageSize, group, code(format),
+                                        code(cacheFormat), StatusWord(), stream_));
+}
+
+void Backend::KVPageGatherInt4(const void *pages, const void *params, const void *pageTable, void *output,
+                               int64_t pageCount, int64_t pageSize, int64_t kvHeads, int64_t headDim, int64_t group,
+                               int64_t outRows, DType format) {
+    Check(puter_hip_kv_page_gather_int4(pages, params, static_cast<const int32_t *>(pageTable), output, pageCount,
+                                        pageSize, kvHeads, headDim, group, outRows, code(format), StatusWord(),
+                                        stream_));
+}
+
 // ---- attention -------------------------------------------------------------------------------
 void Backend::MultiHeadAttention(const MultiHeadAttentionConfig &config, const void *query, const void *key,
                                  const void *value, void *output, int64_t seqQ, int64_t seqK, DType format) {
@@ -342,6 +371,17 @@ void Backend::MultiHeadAttentionBatched(const MultiHeadAttentionConfig &config, 
     const puter_mha_config c = mha_config(config);
     Check(puter_hip_multi_head_attention_batched(&c, query, key, value, output, batch, seqQ, seqK, code(format),
                                                  stream_));
+}
+
+void Backend::MultiHeadAttentionPacked(const MultiHeadAttentionConfig &config, const void *query, const void *key,
+                                       const void *value, void *output, const void *queryOffsets,
+                                       const void *keyOffsets, int64_t batch, int64_t totalQ, int64_t totalK,
+                                       DType format) {
+    const puter_mha_config c = mha_config(config);
+    Check(puter_hip_multi_head_attention_packed(&c, query, key, value, output,
+                                                static_cast<const int32_t *>(queryOffsets),
+                                                static_cast<const int32_t *>(keyOffsets), batch, totalQ, totalK,
+                                                code(format), StatusWord(), stream_));
 }
 
 void Backend::ScaledDotProductAttention(const FlashAttentionConfig &config, const void *query, const void *key,
@@ -375,6 +415,24 @@ void Backend::PagedDecodeAttention(const void *query, const void *keyPages, cons
                                            pageSize, numPages, numHeads, kvHeads, headDim, maxContext,
                                            static_cast<const float *>(kScale), static_cast<const float *>(vScale),
                                            code(kvFormat), output, workspace, workspaceBytes, stream_));
+}
+
+size_t Backend::PagedInt4WorkspaceBytes(int64_t batch, int64_t queryLen, int64_t numHeads, int64_t kvHeads,
+                                        int64_t headDim, int64_t maxContext) {
+    return puter_hip_paged_int4_workspace_bytes(batch, queryLen, numHeads, kvHeads, headDim, maxContext);
+}
+
+void Backend::PagedInt4Attention(const void *query, const void *keyPages, const void *valuePages,
+                                 const void *keyParams, const void *valueParams, const void *pageTable,
+                                 const void *contextLens, int64_t batch, int64_t queryLen, int64_t maxPagesPerSeq,
+                                 int64_t pageSize, int64_t numPages, int64_t numHeads, int64_t kvHeads,
+                                 int64_t headDim, int64_t group, int64_t maxContext, DType format, void *output,
+                                 void *workspace, size_t workspaceBytes) {
+    Check(puter_hip_paged_int4_attention(query, keyPages, valuePages, keyParams, valueParams,
+                                         static_cast<const int32_t *>(pageTable),
+                                         static_cast<const int32_t *>(contextLens), batch, queryLen, maxPagesPerSeq,
+                                         pageSize, numPages, numHeads, kvHeads, headDim, group, maxContext,
+                                         code(format), output, workspace, workspaceBytes, stream_));
 }
 
 // ---- quantisation, matmul ---------------------------------------------------------------------

@@ -239,6 +239,18 @@ public:
                         int64_t pageCount, int64_t pageSize, int64_t kvHeads, int64_t headDim, int64_t valueRows,
                         int64_t storageOffset, const void *scales, DType valueFormat);
 
+    // extension hooks: RoPE of Q and K with the page write of K and V (config nullptr: no
+    // rotation; cacheFormat: format, Float8E4M3 or Int4), and the gather of 4-bit pages as values
+    void KVPageAppendRoPE(const RoPEConfig *config, const void *query, const void *key, const void *value,
+                          const void *positions, const void *pageIDs, const void *offsets, void *queryOut,
+                          void *keyPages, void *valuePages, void *keyParams, void *valueParams, int64_t rows,
+                          int64_t queryHeads, int64_t kvHeads, int64_t headDim, int64_t queryStride,
+                          int64_t keyStride, int64_t valueStride, int64_t pageCount, int64_t pageSize,
+                          int64_t group, DType format, DType cacheFormat);
+    void KVPageGatherInt4(const void *pages, const void *params, const void *pageTable, void *output,
+                          int64_t pageCount, int64_t pageSize, int64_t kvHeads, int64_t headDim, int64_t group,
+                          int64_t outRows, DType format);
+
     // -- Attention: device/interface.go:91-110
     void MultiHeadAttention(const MultiHeadAttentionConfig &config, const void *query, const void *key,
                             const void *value, void *output, int64_t seqQ, int64_t seqK, DType format);
@@ -246,6 +258,11 @@ public:
     void MultiHeadAttentionBatched(const MultiHeadAttentionConfig &config, const void *query, const void *key,
                                    const void *value, void *output, int64_t batch, int64_t seqQ, int64_t seqK,
                                    DType format);
+    // extension: sequences of different lengths back to back, parted by device offsets
+    void MultiHeadAttentionPacked(const MultiHeadAttentionConfig &config, const void *query, const void *key,
+                                  const void *value, void *output, const void *queryOffsets,
+                                  const void *keyOffsets, int64_t batch, int64_t totalQ, int64_t totalK,
+                                  DType format);
     void ScaledDotProductAttention(const FlashAttentionConfig &config, const void *query, const void *key,
                                    const void *value, void *output, int64_t seqQ, int64_t seqK, int64_t depth,
                                    int64_t valueDim, DType format);
@@ -260,6 +277,16 @@ public:
                               int64_t kvHeads, int64_t headDim, int64_t maxContext, const void *kScale,
                               const void *vScale, DType kvFormat, void *output, void *workspace,
                               size_t workspaceBytes);
+
+    // extension: one or a few query tokens per sequence over 4-bit pages
+    size_t PagedInt4WorkspaceBytes(int64_t batch, int64_t queryLen, int64_t numHeads, int64_t kvHeads,
+                                   int64_t headDim, int64_t maxContext);
+    void PagedInt4Attention(const void *query, const void *keyPages, const void *valuePages,
+                            const void *keyParams, const void *valueParams, const void *pageTable,
+                            const void *contextLens, int64_t batch, int64_t queryLen, int64_t maxPagesPerSeq,
+                            int64_t pageSize, int64_t numPages, int64_t numHeads, int64_t kvHeads,
+                            int64_t headDim, int64_t group, int64_t maxContext, DType format, void *output,
+                            void *workspace, size_t workspaceBytes);
 
     // -- Dequant / Quant: device/interface.go:196-199,580-582
     void Dequant(void *dst, const void *src, int64_t count, const DequantInt8Config &config, DType dstFormat,
