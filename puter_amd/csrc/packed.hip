@@ -4,9 +4,10 @@
 // batch of other lengths needs no host synchronisation.  Per sequence the masks are
 // MultiHeadAttention's: key k is visible to query q iff k <= q + seqK - seqQ (causal) and
 // q - k < window, scores scaled by 1/sqrt(D), ALiBi added; a query that sees no key is zero.
-#include "attention.hpp"
+#include "prefill.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace puter {
 
@@ -32,6 +33,179 @@ __device__ __forceinline__ void packed_check(const int32_t *off, int64_t batch, 
     if (!status) return;
     for (int64_t i = threadIdx.x; i < batch; i += blockDim.x)
         if (off[i] < 0 || off[i + 1] < off[i] || off[i + 1] > total) *status = PUTER_ERR_INVALID;
+}
+
+// The MFMA prefill kernels (prefill.hpp) over packed sequences: PrefillArgs whose map finds the
+// block's sequence and sets the arguments to that sequence.
+struct PackedArgs : PrefillArgs {
+    const int32_t *qoff, *koff;
+    int32_t *status;
+    int total_q, total_k, elem;   // elem: bytes of an element
+};
+
+constexpr int kPackedLanes = 256;   // sequences that a wave ranks by length, four a lane
+
+__device__ __forceinline__ int packed_wave_sum(int v) {   // in every lane
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8: sums of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31: of 32, of 64
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The rank-th query tile of the call and its sequence.  Up to 256 sequences the tiles are ranked
+// by how far down their sequence's keys they reach (their level: under a causal mask, their work),
+// the longest first, as the batched kernel starts its heaviest blocks first: F(t), the tiles of
+// level t or more, is one pass over the lanes, and the level where F passes the rank is found by
+// bisection.  More sequences go in their order: sequence i's tiles start at slot
+// floor(offset / 128) + i, which leaves room for each one's last tile.
+__device__ __forceinline__ bool packed_tile(const PackedArgs &a, int rank, int &seq, int &tile) {
+    const int lane = threadIdx.x & 63;
+    if (a.batch > kPackedLanes) {
+        int lo = 0, hi = a.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (min(max(a.qoff[mid], 0), a.total_q) / fa::BM + mid <= rank) lo = mid;
+            else hi = mid;
+        }
+        const int start = min(max(a.qoff[lo], 0), a.total_q);
+        seq = lo;
+        tile = rank - (start / fa::BM + lo);
+        return tile >= 0;
+    }
+    int base[4], n[4], top = 0;   // per sequence: the level of its first tile, its tiles
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        base[c] = n[c] = 0;
+        const int i = 64 * c + lane;
+        if (64 * c >= a.batch) continue;
+        if (i < a.batch) {
+            int64_t q0, q1, k0, k1;
+            packed_range(a.qoff, i, a.total_q, q0, q1);
+            packed_range(a.koff, i, a.total_k, k0, k1);
+            n[c] = (int)((q1 - q0 + fa::BM - 1) / fa::BM);
+            base[c] = (int)max((int64_t)0, (k1 - k0) - (q1 - q0)) / fa::BM;
+        }
+        top = max(top, base[c] + n[c]);
+    }
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+    top = __builtin_amdgcn_readfirstlane(top);
+    auto from_level = [&](int t) __attribute__((always_inline)) {
+        int f = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (64 * c < a.batch) f += min(max(base[c] + n[c] - t, 0), n[c]);
+        return packed_wave_sum(f);
+    };
+    if (rank >= from_level(0)) return false;
+    int lo = 0, hi = top;   // F(lo) > rank >= F(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (from_level(mid) > rank) lo = mid;
+        else hi = mid;
+    }
+    int j = rank - from_level(lo + 1);   // the j-th sequence with a tile of this level
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint64_t have = __ballot(lo >= base[c] && lo < base[c] + n[c]);
+        const int count = __builtin_popcountll(have);
+        if (j < count) {
+            const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0u));
+            const uint64_t mine = __ballot(((have >> lane) & 1) && before == j);
+            const int at = __builtin_ctzll(mine);
+            seq = 64 * c + at;
+            tile = lo - __builtin_amdgcn_readlane(base[c], at);
+            return true;
+        }
+        j -= count;
+    }
+    return false;   // (offsets that fall: fewer tiles than they seemed)
+}
+
+// Block -> (tile, kv head, head of its group): eight (tile, kv head) pairs at a time, one to an
+// XCD, the group's heads one after another there, so a sequence's keys of one kv head are read by
+// one XCD (by few, with fewer kv heads than XCDs).
+__device__ __forceinline__ bool prefill_map(PackedArgs &a, int &qt, int &b, int &h) {
+    const int id = blockIdx.x, G = a.heads / a.kv_heads;
+    if (id == 0) {
+        packed_check(a.qoff, a.batch, a.total_q, a.status);
+        packed_check(a.koff, a.batch, a.total_k, a.status);
+    }
+    const int pair = (id / (8 * G)) * 8 + (id & 7), slot = (id >> 3) % G;
+    int seq = 0;
+    if (!packed_tile(a, pair / a.kv_heads, seq, qt)) return false;
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    qt = __builtin_amdgcn_readfirstlane(qt);
+    h = (pair % a.kv_heads) * G + slot;
+    b = 0;
+    int64_t q0, q1, k0, k1;
+    packed_range(a.qoff, seq, a.total_q, q0, q1);
+    packed_range(a.koff, seq, a.total_k, k0, k1);
+    q0 = __builtin_amdgcn_readfirstlane((int)q0), q1 = __builtin_amdgcn_readfirstlane((int)q1);
+    k0 = __builtin_amdgcn_readfirstlane((int)k0), k1 = __builtin_amdgcn_readfirstlane((int)k1);
+    a.seq_q = (int)(q1 - q0);
+    a.seq_k = (int)(k1 - k0);
+    if (qt >= (a.seq_q + fa::BM - 1) / fa::BM) return false;
+    a.shift = a.seq_k - a.seq_q;
+    const int64_t qrow = (int64_t)a.heads * a.dim * a.elem, krow = (int64_t)a.kv_heads * a.dim * a.elem;
+    a.q = reinterpret_cast<const uint16_t *>(reinterpret_cast<const char *>(a.q) + q0 * qrow);
+    a.o = reinterpret_cast<uint16_t *>(reinterpret_cast<char *>(a.o) + q0 * qrow);
+    a.k = reinterpret_cast<const uint16_t *>(reinterpret_cast<const char *>(a.k) + k0 * krow);
+    a.v = reinterpret_cast<const uint16_t *>(reinterpret_cast<const char *>(a.v) + k0 * krow);
+    return true;
+}
+
+// 16-bit head dims of 8 n and f32 head dims of 4 n, 16-byte aligned; false: the row kernel's.
+static bool launch_packed_mfma(const PackedMha &m, int dtype, hipStream_t s) {
+    const bool f32 = dtype == PUTER_F32;
+    if (m.dim % (f32 ? 4 : 8)) return false;
+    if (m.kv_heads * m.dim > (f32 ? 32768 : 65536) * 128) return false;   // a K/V tile spans < 2^30 bytes
+    if (!aligned16(m.q) || !aligned16(m.k) || !aligned16(m.v) || !aligned16(m.o)) return false;
+    if (m.total_k >= ((int64_t)1 << 30)) return false;
+    // ranks: every sequence's last tile may be a part of one
+    const int64_t tiles = m.total_q / fa::BM + std::min(m.batch, m.total_q), G = m.heads / m.kv_heads;
+    const int64_t ranks = m.batch > kPackedLanes ? m.total_q / fa::BM + m.batch : tiles;
+    const int64_t blocks = (ranks * m.kv_heads + 7) / 8 * 8 * G;
+    if (blocks > 0x7FFFFFFF) return false;
+    PackedArgs a{};
+    a.q = static_cast<const uint16_t *>(m.q);
+    a.k = static_cast<const uint16_t *>(m.k);
+    a.v = static_cast<const uint16_t *>(m.v);
+    a.o = static_cast<uint16_t *>(m.o);
+    a.batch = (int)m.batch;
+    a.heads = (int)m.heads;
+    a.kv_heads = (int)m.kv_heads;
+    a.dim = (int)m.dim;
+    a.nan_rows = 1;
+    a.causal = m.causal;
+    a.window = (int)std::min<int64_t>(m.window, 0x3FFFFFFF);
+    a.alibi_s = m.alibi != 0.0f ? m.alibi / m.scale : 0.0f;
+    a.scale_log2 = m.scale * 1.4426950408889634f;
+    if (f32 && m.dim != 64 && m.dim != 128) {   // as launch_prefill_f32
+        const double exact = (double)m.scale * 1.4426950408889634;
+        a.scale_log2 = (float)exact;
+        if ((double)a.scale_log2 >= exact) a.scale_log2 = std::nextafter(a.scale_log2, 0.0f);
+        a.scale_log2_lo = (float)(exact - (double)a.scale_log2);
+    }
+    a.qoff = m.qoff, a.koff = m.koff, a.status = m.status;
+    a.total_q = (int)m.total_q, a.total_k = (int)m.total_k, a.elem = f32 ? 4 : 2;
+    const bool gen = a.window > 0 || a.alibi_s != 0.0f;
+    const dim3 grid((unsigned)blocks);
+    with_head_dim(m.dim, [&](auto d) {
+        if (f32) {
+            if (gen) prefill_f32_kernel<d.D, true, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
+            else prefill_f32_kernel<d.D, false, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
+        } else if (dtype == PUTER_BF16) {
+            if (gen) prefill_kernel<PUTER_BF16, d.D, true, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
+            else prefill_kernel<PUTER_BF16, d.D, false, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
+        } else {
+            if (gen) prefill_kernel<PF_F16_DOT32, d.D, true, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
+            else prefill_kernel<PF_F16_DOT32, d.D, false, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
+        }
+    });
+    return true;
 }
 
 // Any dtype, head dim up to 256 and alignment: a wave per query row and head.  Lanes take 64
@@ -132,6 +306,7 @@ extern "C" int puter_hip_multi_head_attention_packed(const puter_mha_config *con
                 H, kvh, D, config->causal ? 1 : 0, config->window_size, config->alibi_slope,
                 (float)(1.0 / sqrt((double)D)), status};
     hipStream_t s = as_stream(stream);
+    if (launch_packed_mfma(a, dtype, s)) return check_launch("mha packed mfma");
     const dim3 grid((unsigned)total_q, (unsigned)H);
     switch (dtype) {
     case PUTER_F32: mha_packed_row_kernel<PUTER_F32><<<grid, 64, 0, s>>>(a); break;

@@ -744,16 +744,17 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_kernel(Args a) {
     __shared__ __attribute__((aligned(1024))) char k1s[T::TILE];
     __shared__ __attribute__((aligned(1024))) char v0s[T::TILE];
     __shared__ __attribute__((aligned(1024))) char v1s[T::TILE];
-    __shared__ int redo;   // PAD: bit w: some output of dims 64 w .. + 63 is not finite
+    // packed sequences also get the second walk at 64 and 128 dims: what a mask hides has no effect there
+    constexpr bool PACKED = !std::is_same<Args, PrefillArgs>::value, REDO = PAD || PACKED;
+    __shared__ int redo;   // REDO: bit w: some output of dims 64 w .. + 63 is not finite
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, g = lane >> 5;
-    if (PAD && tid == 0) redo = 0;
+    if (REDO && tid == 0) redo = 0;
 
     int qt, b, h;
     if (!prefill_map(a, qt, b, h)) return;
-    constexpr bool PACKED = !std::is_same<Args, PrefillArgs>::value;
     const int kvh = h / (a.heads / a.kv_heads);
     const int q0 = qt * BM;
     const int dim = PAD ? a.dim : D;
@@ -857,7 +858,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_kernel(Args a) {
     const float inv = ltot > 0.0f ? 1.0f / ltot : 0.0f;
     uint32_t bits[(T::DB + 1) / 2] = {};
     bool spoiled = false;
-    if constexpr (PAD) {
+    if constexpr (REDO) {
         spoiled = ltot > 0.0f && qi < a.seq_q && prefill_spoiled(st.o, bits);
         if (spoiled) {
 #pragma unroll
@@ -882,11 +883,11 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_kernel(Args a) {
                 if (32 * d + 8 * rb >= dim) continue;   // dim % 8 == 0: an 8-dim run is whole or absent
                 V4 v;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = (E)(PAD && !(ltot > 0.0f) ? st.o[d][4 * rb + i] : st.o[d][4 * rb + i] * inv);
+                for (int i = 0; i < 4; ++i) v[i] = (E)(REDO && !(ltot > 0.0f) ? st.o[d][4 * rb + i] : st.o[d][4 * rb + i] * inv);
                 *reinterpret_cast<V4 *>(orow + 32 * d + 8 * rb + 4 * g) = v;
             }
     }
-    if constexpr (PAD) {
+    if constexpr (REDO) {
         __syncthreads();
         if (__builtin_expect(!redo, 1)) return;
         // (the lane and its offsets afresh, so that none of them is alive for this in the first walk)
@@ -1029,16 +1030,17 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_f32_kernel(Args 
     __shared__ __attribute__((aligned(1024))) char k1s[T::TILE];
     __shared__ __attribute__((aligned(1024))) char v0s[T::TILE];
     __shared__ __attribute__((aligned(1024))) char v1s[T::TILE];
-    __shared__ int redo;   // PAD: bit w: some output of dims 64 w .. + 63 is not finite
+    // packed sequences also get the second walk at 64 and 128 dims: what a mask hides has no effect there
+    constexpr bool PACKED = !std::is_same<Args, PrefillArgs>::value, REDO = PAD || PACKED;
+    __shared__ int redo;   // REDO: bit w: some output of dims 64 w .. + 63 is not finite
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h = lane >> 5;
-    if (PAD && tid == 0) redo = 0;
+    if (REDO && tid == 0) redo = 0;
 
     int qt, b, hd;
     if (!prefill_map(a, qt, b, hd)) return;
-    constexpr bool PACKED = !std::is_same<Args, PrefillArgs>::value;
     const int kvh = hd / (a.heads / a.kv_heads);
     const int q0 = qt * BM;
     const float *const qp = reinterpret_cast<const float *>(a.q);
@@ -1253,17 +1255,21 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_f32_kernel(Args 
     const float ltot = swap_halves_sum(l);
     uint32_t bits[(T::DB + 1) / 2] = {};
     bool spoiled = false;
-    if constexpr (PAD) {
+    if constexpr (REDO) {
         spoiled = ltot > 0.0f && qi < a.seq_q && prefill_spoiled(o, bits);
         if (spoiled) {
 #pragma unroll
             for (int w = 0; w < (T::DB + 1) / 2; ++w)
                 if (bits[w]) atomicOr(&redo, 1 << w);
         }
-        if (!(ltot > 0.0f)) {   // a NaN score: zeros, as the general kernel
+        if (!(ltot > 0.0f)) {   // a NaN score: zeros, as the general kernel (packed: NaN)
+            const float z = PACKED && a.nan_rows ? ltot : 0.0f;
 #pragma unroll
-            for (int db = 0; db < 8; ++db)
-                if (db < T::DB) o[db] = (f32x16){};
+            for (int db = 0; db < 8; ++db) {
+                if (db >= T::DB) break;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] = z;
+            }
         }
     }
     float *orow;
@@ -1289,7 +1295,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_f32_kernel(Args 
         }
     } else {
         // normalise and store: lane holds O[qi][32 db + 8 (r/4) + 4 h + r%4]
-        inv = ltot > 0.0f ? 1.0f / ltot : 0.0f;
+        inv = ltot > 0.0f ? 1.0f / ltot : PACKED ? 1.0f : 0.0f;
         orow = reinterpret_cast<float *>(a.o) + (int64_t)b * a.seq_q * qrs + (int64_t)qi * qrs + (int64_t)hd * dim;
         if (qi < a.seq_q) {
 #pragma unroll
@@ -1306,7 +1312,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_f32_kernel(Args 
             }
         }
     }
-    if constexpr (PAD) {   // outputs that are not finite, once they are stored
+    if constexpr (REDO) {   // outputs that are not finite, once they are stored
         __syncthreads();
         if (!redo) return;
         const float *qrow = qbase + (int64_t)min(qi, a.seq_q - 1) * qrs;
