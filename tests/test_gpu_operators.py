@@ -543,11 +543,19 @@ def check_int4_attention(out, s, m, page, f, d, max_context=None, bad_pages=()):
                 keep[i * page:(i + 1) * page] = False
                 ids[i] = 0
         k, v = (int4_values(s[x + "c"][ids], s[x + "p"][ids]).flatten(0, 1)[:n] for x in "kv")
+        part = s["vp"][ids].clone()
+        part[..., 1] = 0
+        codes = int4_values(s["vc"][ids], part).flatten(0, 1)[:n]   # the values without their offsets
         for i in range(m):   # each query with the keys it sees
             mine = keep & (torch.arange(n) <= n - m + i)
             ref, mag, top = attend(s["q"][b, i:i + 1].double(), k[mine], v[mine], 0, causal=False)
             # the code products and the offset sums cancel: terms up to 24 steps beside the value's 8 and offset
-            within(out[b, i:i + 1], ref, attention_bound(f, ref, 6 * mag + 1e-3 * mag.max(), 6 * top, d, max(n, 1), 2.0 ** -16), f"sequence {b}, query {i}")
+            bound = attention_bound(f, ref, 6 * mag + 1e-3 * mag.max(), 6 * top, d, max(n, 1), 2.0 ** -16)
+            # P is scaled by the token's scale and rounded once to bf16 for bf16 outputs, half a step, before
+            # it meets the code: off by at most H sum p |scale n| (the offsets meet p itself)
+            if f == BF16:
+                bound += H(f) * (1 + H(f)) * attend(s["q"][b, i:i + 1].double(), k[mine], codes[mine], 0, causal=False)[1]
+            within(out[b, i:i + 1], ref, bound, f"sequence {b}, query {i}")
 
 
 INT4 = [
