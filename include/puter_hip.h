@@ -309,6 +309,7 @@ PUTER_API int puter_hip_kv_page_write_fp8(void *storage, const void *values, con
  *     scale = f16((hi - lo) / 15), offset = f16((lo + hi) / 2 + scale / 2), nibble =
  *     rint((x - offset) * (1 / scale)) in [-8, 7], 0 where scale is 0; a NaN makes its
  *     group's scale and offset NaN.  Pools 16-byte aligned.
+ * The angles are kept to 2^45 radians: a start or a base that can pass that is refused.
  * Ids, slots, *status and several rows of one slot as puter_hip_kv_page_write; the query
  * of a row that is not stored is still written.  head_dim: even, at most 1024. */
 PUTER_API int puter_hip_kv_page_append_rope(const puter_rope_config *config, const void *query, const void *key,
@@ -322,7 +323,8 @@ PUTER_API int puter_hip_kv_page_append_rope(const puter_rope_config *config, con
 
 /* Extension: KVPageGather of a 4-bit pool as values: output [out_rows, kv_heads *
  * head_dim] of dtype (F32, F16, BF16), row i from page page_table[i / page_size], slot
- * i % page_size.  A bad id gives a zero row and *status, as puter_hip_kv_page_gather. */
+ * i % page_size.  A bad id gives a zero row and *status, as puter_hip_kv_page_gather.
+ * out_rows and page_size below 2^31. */
 PUTER_API int puter_hip_kv_page_gather_int4(const void *pages, const void *params, const int32_t *page_table,
                                             void *output, int64_t page_count, int64_t page_size, int64_t kv_heads,
                                             int64_t head_dim, int64_t group, int64_t out_rows, int dtype,

@@ -198,6 +198,30 @@ def test_append_is_rope_and_page_write(backend, f, mode):
     assert torch.equal(s["pools"][1].cpu()[at], want[1].cpu()[at])
 
 
+@pytest.mark.parametrize("f", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,dim", [(70, 64), (70, 20), (1500, 64)])
+def test_append_fp8_bytes_are_the_page_write_s(backend, f, rows, dim):
+    """Unrotated rows into fp8 pages: byte for byte what KVPageWriteFP8 stores, whatever the scale
+    (least, zero, negative, vast, not a number) and the value (ties, infinities, NaN)."""
+    scales = torch.tensor([1.0, 0.0078, 3.0, 1e-42, 0.0, 2.0 ** -60, 2.0 ** -61, 1e30, -0.5, math.inf, math.nan, 3e38]).cuda()
+    kvh, page = len(scales), 16
+    s = append_state(rows, 1, kvh, dim, f, E4M3, 0, page, False, seed=21)
+    k = s["dev"][1]
+    grid = torch.arange(rows * dim, device="cuda").view(rows, dim)
+    tie = ((grid % 127) + 8.5) / 16 * torch.exp2((grid % 23 - 12).float())    # half steps of the format
+    for h in range(kvh):
+        k[:, h] = (tie * (scales[h] if torch.isfinite(scales[h]) else 1.0)).clamp(-3e38, 3e38).to(T[f])
+    k[0, :, :4] = torch.tensor([math.inf, -math.inf, math.nan, 0.0], device="cuda").to(T[f])
+    s["par"] = [scales, scales.flip(0).contiguous()]
+    want = [p.clone() for p in s["pools"]]
+    call_append(backend, None, s, rows, 1, kvh, dim, f, E4M3, 0, page)
+    for w, x, p in zip(want, s["dev"][1:], s["par"]):
+        backend.KVPageWriteFP8(w, x, s["ids"].cuda(), s["slots"].cuda(), s["pages"], page, kvh, dim, rows, 0, p, f)
+    backend.CheckStatus()
+    for got, w in zip(s["pools"], want):
+        assert torch.equal(got, w)
+
+
 def test_append_without_rotation(backend):
     rows, kvh, dim, page = 10, 2, 64, 4
     s = append_state(rows, 3, kvh, dim, BF16, BF16, 0, page, True, seed=8)
@@ -481,6 +505,21 @@ def test_packed_bad_offsets_are_reported(backend, f, d):
     within(out[10:30], ref, attention_bound(f, ref, mag, top, d, 20, p_bits(f)))
 
 
+def test_packed_rows_past_4_gib(backend):
+    """Queries and outputs that pass 2^32 bytes: the last sequence's rows."""
+    h, kv, d, f, n, b = 32, 2, 128, BF16, 1000, 530
+    q = torch.randn((n * b, h, d), dtype=T[f], device="cuda")
+    k, v = (torch.randn((n * b, kv, d), dtype=T[f], device="cuda") for _ in range(2))
+    off = torch.arange(b + 1, dtype=torch.int32, device="cuda") * n
+    out = torch.zeros_like(q)
+    call_packed(backend, q, k, v, out, off, None, h, kv, d, f)
+    backend.CheckStatus()
+    for at in (0, (b - 1) * n):
+        rows = slice(at, at + n)
+        ref, mag, top = attend(q[rows].double().cpu(), k[rows].double().cpu(), v[rows].double().cpu(), 0)
+        within(out[rows], ref, attention_bound(f, ref, mag, top, d, n, p_bits(f)), at)
+
+
 def test_packed_unaligned(backend):
     lens, h, kv, d = [40, 70], 2, 2, 64
     q, k, v, off = packed_state(lens, lens, h, kv, d, BF16)
@@ -556,6 +595,37 @@ def check_int4_attention(out, s, m, page, f, d, max_context=None, bad_pages=()):
             if f == BF16:
                 bound += H(f) * (1 + H(f)) * attend(s["q"][b, i:i + 1].double(), k[mine], codes[mine], 0, causal=False)[1]
             within(out[b, i:i + 1], ref, bound, f"sequence {b}, query {i}")
+
+
+def test_4_bit_pools_past_4_gib(backend):
+    """Append, gather and attention on a page whose codes lie past 2^32 bytes of the pool."""
+    h, kv, d, group, page, n, f = 4, 2, 128, 64, 16, 40, BF16
+    pages = (1 << 32) // (page * kv * d // 2) + 8
+    pools = [torch.empty((pages, page, kv, d // 2), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    par = [torch.empty((pages, page, kv, d // group, 2), dtype=torch.float16, device="cuda") for _ in range(2)]
+    table = torch.tensor([[pages - 1, pages - 3, pages - 2]], dtype=torch.int32)
+    q, k, v = (randn(60 + i, (n, x, d), f).cuda() for i, x in enumerate((h, kv, kv)))
+    t = torch.arange(n, dtype=torch.int32)
+    backend.KVPageAppendRoPE(None, None, k, v, None, table[0][(t // page).long()].cuda(), (t % page).cuda(), None, pools[0], pools[1],
+                             par[0], par[1], n, 0, kv, d, 0, kv * d, kv * d, pages, page, group, f, I4)
+    last = slice(pages - 4, pages)
+    s = {"table": table - (pages - 4), "ctx": torch.tensor([n], dtype=torch.int32), "q": q.cpu()[-1:].unsqueeze(1)}
+    for x, c, p in zip("kv", pools, par):
+        s[x + "c"], s[x + "p"] = c[last].cpu(), p[last].cpu()
+        out = torch.empty((n, kv, d), dtype=T[f], device="cuda")
+        backend.KVPageGatherInt4(c, p, table.cuda(), out, pages, page, kv, d, group, n, f)
+        ids = s["table"][0].long()
+        val = int4_values(s[x + "c"][ids], s[x + "p"][ids]).flatten(0, 1)[:n]
+        within(out, val, H(f) * val.abs() + 2 * U * (val.abs() + 16), "gather")   # a product and a sum, terms below 16
+    for i, x in enumerate((k, v)):
+        check_int4(s["kv"[i] + "c"][ids].flatten(0, 1)[:n], s["kv"[i] + "p"][ids].flatten(0, 1)[:n], x.double().cpu(),
+                   torch.zeros(x.shape, dtype=torch.float64), group, "kv"[i])
+    need = backend.PagedInt4WorkspaceBytes(1, 1, h, kv, d, n)
+    ws, o = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.zeros((1, 1, h, d), dtype=T[f], device="cuda")
+    backend.PagedInt4Attention(q[-1:], pools[0], pools[1], par[0], par[1], table.cuda(), s["ctx"].cuda(), 1, 1, 3, page, pages, h, kv, d,
+                               group, n, f, o, ws, need)
+    backend.CheckStatus()
+    check_int4_attention(o, s, 1, page, f, d)
 
 
 INT4 = [

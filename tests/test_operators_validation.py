@@ -1,6 +1,7 @@
 """CPU: what the packed attention, the appending page write and the 4-bit cache's calls refuse,
 before any launch (no pointer is read here)."""
 import ctypes as C
+import math
 
 import pytest
 
@@ -45,6 +46,9 @@ def append(lib, **kw):
     dict(kpages=FAKE + 8), dict(vpages=FAKE + 4), dict(kpar=FAKE + 2), dict(vpar=FAKE + 1), dict(status=FAKE + 2),
     dict(config=rope(base_freq=0.0)), dict(config=rope(mode=2)), dict(config=rope(scaling=2)),
     dict(config=rope(scaling=1, scaling_factor=8.0, low_freq_factor=4.0, high_freq_factor=1.0, original_context=8)),
+    dict(config=rope(base_freq=math.inf)), dict(config=rope(base_freq=math.nan)), dict(config=rope(start_position=1 << 46)),
+    dict(config=rope(start_position=-(1 << 62))), dict(config=rope(base_freq=1e-9)),
+    dict(config=rope(scaling=1, scaling_factor=1e-5, low_freq_factor=1.0, high_freq_factor=4.0, original_context=8)),
     dict(qh=70000, qs=70000 * 128), dict(kvh=70000, ks=70000 * 128, vs=70000 * 128),
 ])
 def test_append_refuses(lib, change):
@@ -71,7 +75,7 @@ GATHER = dict(pages=FAKE, params=FAKE, table=FAKE, out=FAKE, count=4, page_size=
 def test_gather_refuses(lib):
     def call(**kw):
         return lib.puter_hip_kv_page_gather_int4(*dict(GATHER, **kw).values())
-    for change in (dict(dtype=I4), dict(dtype=E4M3), dict(count=-1), dict(page_size=0), dict(kvh=0), dict(rows=-1),
+    for change in (dict(dtype=I4), dict(dtype=E4M3), dict(count=-1), dict(page_size=0), dict(page_size=1 << 31), dict(kvh=0), dict(rows=-1), dict(rows=1 << 31),
                    dict(dim=80), dict(group=48), dict(dim=64, group=128), dict(pages=FAKE + 2), dict(params=FAKE + 1),
                    dict(status=FAKE + 3), dict(kvh=70000), dict(rows=1 << 60)):
         assert call(**change) == _lib.ERR_INVALID, change
