@@ -26,13 +26,14 @@
  *     head dim 128 without ALiBi, or any row over more than 768 keys) or in F32
  *     with at least 16 query rows, a head dim that is a multiple of 4, and
  *     fewer 128-query blocks than two per CU (causal) or one per CU (not
- *     causal): four buffers per device (the default stream's and one for all
+ *     causal), and puter_hip_multi_head_attention_packed in F32 with fewer
+ *     than two per CU: four buffers per device (the default stream's and one for all
  *     other streams, each once for calls that also run on scratch under capture
  *     and once for those that do not), allocated on first use and grown on
  *     demand (Matmul: at most 16 MiB, 96 MiB for 256x256 tiles; one-row attention: the paged decode
  *     workspace size, or batch x heads x ceil(seq_k / 256) x (head_dim + 2)
- *     floats; F32 attention: key splits x batch x seq_q x heads x (head_dim +
- *     2) floats, at most about 100 MB; scaled-dot-product attention: see there).
+ *     floats; F32 attention: key splits x batch x seq_q (or total_q) x heads x
+ *     (head_dim + 2) floats, at most about 100 MB (packed 140 MB); scaled-dot-product attention: see there).
  *     A growth is stream-ordered on the calling
  *     stream (hipFreeAsync of the old buffer after its last user, then
  *     hipMallocAsync): it never blocks the host.  On a stream that is capturing
@@ -428,7 +429,8 @@ PUTER_API int puter_hip_paged_decode_attention(const void *query, const void *ke
  * context_lens[b] tokens (clamped to max_context), the last query_len of them its queries'
  * own: query i sees the tokens up to context - query_len + i, and gives zeros where there
  * is none.  page_table [batch, max_pages_per_seq]; a token whose page id is outside [0,
- * num_pages) is masked, never read.  num_heads any multiple of kv_heads.  query, output,
+ * num_pages) is masked, never read.  A pair that is not finite makes what it enters NaN
+ * for the rows that see its token (a V pair: its group of dims) and no other.  num_heads any multiple of kv_heads.  query, output,
  * pools, pairs and workspace 16-byte aligned; workspace: caller-owned,
  * puter_hip_paged_int4_workspace_bytes(...) bytes of any content, used by one call at a time. */
 PUTER_API size_t puter_hip_paged_int4_workspace_bytes(int64_t batch, int64_t query_len, int64_t num_heads,

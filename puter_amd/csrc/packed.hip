@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <optional>
 
 namespace puter {
 
@@ -41,6 +42,9 @@ struct PackedArgs : PrefillArgs {
     const int32_t *qoff, *koff;
     int32_t *status;
     int total_q, total_k, elem;   // elem: bytes of an element
+    int row0;                     // the sequence's first query row (set by the map)
+    // the partials' row of query qi of the sequence in this block's split of the keys
+    __device__ __forceinline__ int64_t part_row(int qi) const { return (int64_t)blockIdx.y * total_q + row0 + qi; }
 };
 
 constexpr int kPackedLanes = 256;   // sequences that a wave ranks by length, four a lane
@@ -149,6 +153,7 @@ __device__ __forceinline__ bool prefill_map(PackedArgs &a, int &qt, int &b, int 
     a.seq_k = (int)(k1 - k0);
     if (qt >= (a.seq_q + fa::BM - 1) / fa::BM) return false;
     a.shift = a.seq_k - a.seq_q;
+    a.row0 = (int)q0;
     const int64_t qrow = (int64_t)a.heads * a.dim * a.elem, krow = (int64_t)a.kv_heads * a.dim * a.elem;
     a.q = reinterpret_cast<const uint16_t *>(reinterpret_cast<const char *>(a.q) + q0 * qrow);
     a.o = reinterpret_cast<uint16_t *>(reinterpret_cast<char *>(a.o) + q0 * qrow);
@@ -157,8 +162,56 @@ __device__ __forceinline__ bool prefill_map(PackedArgs &a, int &qt, int &b, int 
     return true;
 }
 
+// The key splits of the f32 kernel: a thread per four dims of a row and head folds them in order with
+// weights exp2(m_s - M), the loads of four splits at a time.  A split without tiles, or whose keys
+// are all hidden, has m = -inf and adds its sum alone (0, or the NaN of scores that are NaN); its
+// outputs may not have been written and are not used.  Rows outside every sequence have no partials
+// and stay.
+__global__ __launch_bounds__(256) void packed_f32_combine_kernel(PackedArgs a, int splits) {
+    const uint32_t quads = a.dim / 4, id = blockIdx.x * 256 + threadIdx.x, at = id / quads, d = (id - at * quads) * 4;
+    const int64_t rows = (int64_t)a.total_q * a.heads;
+    if (at >= rows) return;
+    const int row = (int)(at / (uint32_t)a.heads);
+    if (row < a.qoff[0] || row >= a.qoff[a.batch]) return;
+    float M = -INFINITY, sum = 0.0f;
+    f32x4 acc = {};
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+        float2 ml[4];
+        f32x4 o[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int s = min(s0 + u, splits - 1);
+            ml[u] = a.part_ml[s * rows + at];
+            o[u] = *reinterpret_cast<const f32x4 *>(a.part_o + (s * rows + at) * a.dim + d);
+        }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (s0 + u < splits) top = fmaxf(top, ml[u].x);
+        const float keep = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - top);
+        if (M != -INFINITY) {   // (a NaN or 0 alone has no weight to change)
+            sum *= keep;
+            acc *= keep;
+        }
+        M = top;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (s0 + u >= splits) break;
+            if (ml[u].x == -INFINITY) {
+                sum += ml[u].y;
+            } else {
+                const float w = __builtin_amdgcn_exp2f(ml[u].x - M);
+                sum += w * ml[u].y;
+                acc += w * o[u];
+            }
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + (int64_t)at * a.dim + d) = acc * inv;
+}
+
 // 16-bit head dims of 8 n and f32 head dims of 4 n, 16-byte aligned; false: the row kernel's.
-static bool launch_packed_mfma(const PackedMha &m, int dtype, hipStream_t s) {
+static bool launch_packed_mfma(const PackedMha &m, int dtype, hipStream_t s, int *status) {
     const bool f32 = dtype == PUTER_F32;
     if (m.dim % (f32 ? 4 : 8)) return false;
     if (m.kv_heads * m.dim > (f32 ? 32768 : 65536) * 128) return false;   // a K/V tile spans < 2^30 bytes
@@ -192,7 +245,31 @@ static bool launch_packed_mfma(const PackedMha &m, int dtype, hipStream_t s) {
     a.qoff = m.qoff, a.koff = m.koff, a.status = m.status;
     a.total_q = (int)m.total_q, a.total_k = (int)m.total_k, a.elem = f32 ? 4 : 2;
     const bool gen = a.window > 0 || a.alibi_s != 0.0f;
-    const dim3 grid((unsigned)blocks);
+    // f32: a block's keys are split over blockIdx.y while there are fewer than two blocks a CU, up to
+    // about two a CU, in runs of two key tiles or more; each block cuts its own tiles, whose number the
+    // host does not know.  2331 rows of five sequences (8 heads of 80, a window of 512): 163 us unsplit,
+    // 74 so, 85 at four splits in place of three, 90 at two; runs of 6 tiles or more lose where
+    // sequences are short (300 rows, 8 heads of 64: 16 us against 24).  The partials lie in the
+    // library's scratch, which cannot grow while a graph is recorded: there the keys stay together.
+    int64_t splits = 1;
+    const int64_t cus = device_cus(), rows = m.total_q * m.heads;
+    if (f32 && blocks < 2 * cus && !scratch_capturing(s)) {
+        const int64_t keys = m.window > 0 ? std::min(m.total_k, m.window + fa::BM) : m.total_k;
+        splits = std::max<int64_t>(1, std::min<int64_t>((2 * cus + blocks - 1) / blocks, keys / 64));
+    }
+    const size_t part = (size_t)(splits * rows * m.dim) * sizeof(float), need = part + (size_t)(splits * rows) * sizeof(float2);
+    std::optional<ScratchLease> lease;
+    if (splits > 1) {
+        lease.emplace(need, s, true);
+        if (lease->status()) {
+            lease.reset();   // no room: unsplit
+            splits = 1;
+        } else {   // outputs first: a multiple of 16 bytes
+            a.part_o = static_cast<float *>(lease->ptr());
+            a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(lease->ptr()) + part);
+        }
+    }
+    const dim3 grid((unsigned)blocks, (unsigned)splits);
     with_head_dim(m.dim, [&](auto d) {
         if (f32) {
             if (gen) prefill_f32_kernel<d.D, true, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
@@ -205,6 +282,12 @@ static bool launch_packed_mfma(const PackedMha &m, int dtype, hipStream_t s) {
             else prefill_kernel<PF_F16_DOT32, d.D, false, d.PAD, PackedArgs><<<grid, 256, 0, s>>>(a);
         }
     });
+    if (lease) packed_f32_combine_kernel<<<(unsigned)((rows * (m.dim / 4) + 255) / 256), 256, 0, s>>>(a, (int)splits);
+    *status = check_launch("mha packed mfma");
+    if (lease) {
+        const int fin = lease->finish();
+        if (!*status) *status = fin;
+    }
     return true;
 }
 
@@ -306,7 +389,8 @@ extern "C" int puter_hip_multi_head_attention_packed(const puter_mha_config *con
                 H, kvh, D, config->causal ? 1 : 0, config->window_size, config->alibi_slope,
                 (float)(1.0 / sqrt((double)D)), status};
     hipStream_t s = as_stream(stream);
-    if (launch_packed_mfma(a, dtype, s)) return check_launch("mha packed mfma");
+    int rc = PUTER_OK;
+    if (launch_packed_mfma(a, dtype, s, &rc)) return rc;
     const dim3 grid((unsigned)total_q, (unsigned)H);
     switch (dtype) {
     case PUTER_F32: mha_packed_row_kernel<PUTER_F32><<<grid, 64, 0, s>>>(a); break;

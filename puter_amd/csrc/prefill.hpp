@@ -1230,6 +1230,17 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_f32_kernel(Args 
         tlo = max(tlo, ylo);
         thi = min(ntiles, ylo + a.split_tiles);
     }
+    if constexpr (PACKED) {   // blockIdx.y's share of this block's own tiles, two or more
+        if (a.part_ml) {
+            const int run = max(2, (ntiles - wlo + (int)gridDim.y - 1) / (int)gridDim.y);
+            tlo = min(ntiles, wlo + (int)blockIdx.y * run);
+            thi = min(ntiles, tlo + run);
+            if (tlo >= thi) {   // none left: nothing but the empty sum is read of it
+                if (qi < a.seq_q && h == 0) a.part_ml[a.part_row(qi) * a.heads + hd] = make_float2(-INFINITY, 0.0f);
+                return;
+            }
+        }
+    }
     if (tlo < thi) copy_tile(tlo * BN, k0s, v0s);
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
     __syncthreads();
@@ -1276,7 +1287,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_f32_kernel(Args 
     float inv = 1.0f;
     if (a.part_ml) {
         // split: the row's (max, sum) and unnormalised output to the partials
-        const int64_t prow = (((int64_t)blockIdx.y * a.batch + b) * a.seq_q + qi) * a.heads + hd;
+        int64_t prow = (((int64_t)blockIdx.y * a.batch + b) * a.seq_q + qi) * a.heads + hd;
+        if constexpr (PACKED) prow = a.part_row(qi) * a.heads + hd;
         orow = a.part_o + prow * dim;
         if (qi < a.seq_q) {
             if (h == 0) a.part_ml[prow] = make_float2(m, ltot);
