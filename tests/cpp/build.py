@@ -12,7 +12,7 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 BIN = os.path.join(HERE, "bin")
-PROGRAMS = {"host_registry_test": False, "host_parity_test": True}   # name -> links the oracle
+PROGRAMS = {"host_registry_test": False, "host_parity_test": True, "host_operators_test": True}   # name -> links the oracle
 
 FLAGS = ["-O2", "-std=c++17", "-Wall", "-Wextra", "-Wno-unused-parameter",
          "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "puter_amd", "host"),
