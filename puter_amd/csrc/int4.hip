@@ -219,6 +219,11 @@ __global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_
     Int4Line line(a, pairs);
     const Int4Cut cut(a.workers, line.total);
     if (worker >= cut.workers) return;
+    // Four neighbouring heads' waves share the lines of a token's row (64 bytes of 128 each at D 128), but
+    // the copies in flight are several times the L1: apart by a step, each fetches the line for itself.
+    // Of one worker, they walk the same steps, so a barrier can keep them together.  64 sequences of 512 to 8192
+    // tokens, 8 kv heads: 79 -> 74 us; runs of a step or two lose 1 %, and go without.
+    const bool together = a.head_group == 4 && cut.each >= 4;
     const int line0 = cut.start(worker);
     int left = cut.start(worker + 1) - line0;
     int ctx;
@@ -433,6 +438,7 @@ __global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_
                 }
                 scaled(3, NG - 1, (4 * NG - 1) & 1);
                 int4_wait_lds();   // K's LDS is read
+                if (together) __builtin_amdgcn_s_barrier();
                 if (more) fetch(a.vp, a.vpar, row1, tk);   // V of the next step into K's tile
                 const bool full = live == ~0ull && 64 * step + 63 <= ctx - a.query_len;
                 uint32_t vis[NT];   // bit 4 i + r: the row sees the token
@@ -629,14 +635,17 @@ __global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_
     }
 }
 
-// Joins a row's pieces: D / 4 threads to a piece, 16 bytes each, the pieces dealt out to the block's
-// groups of D / 4 threads, eight loads of each in flight; the groups' results meet in LDS, in order.
-template <int DT, int D, int NT, int WAVES>
+// Joins a row's pieces: T threads to a piece, 16 bytes each, the pieces dealt out to the block's groups
+// of T threads, eight loads of each in flight; a wave's groups meet by shuffles, the waves in LDS, both in
+// one order.  T = D / 4 in one wave where there are few pieces a row.  Where there are many (three contexts
+// of 50 to 120 thousand tokens leave 340 a row, 174 KB, for 48 rows), one CU cannot read them fast enough:
+// a block for every 32 dims, with eight waves of eight groups, takes 5.6 us, whole rows by eight waves 9.4.
+template <int DT, int D, int NT, int WAVES, int T>
 __global__ __launch_bounds__(64 * WAVES) void int4_join_kernel(Int4Args a) {
-    constexpr int T = D / 4, PG = 64 * WAVES / T, U = 8;   // threads of a piece, groups, loads
-    __shared__ float ml[PG][2];
-    __shared__ float4 os[PG][T];
-    const int h = blockIdx.x, qi = blockIdx.y, b = blockIdx.z;
+    constexpr int CUTS = D / 4 / T, PG = 64 * WAVES / T, U = 8;   // blocks of a row, groups, loads
+    __shared__ float2 ml[WAVES];
+    __shared__ float4 os[WAVES][T];
+    const int h = blockIdx.x / CUTS, cut_at = blockIdx.x % CUTS * T, qi = blockIdx.y, b = blockIdx.z;
     const int2 start = a.starts[b];
     const Int4Cut cut(a.workers, a.starts[a.batch].x);
     const int G = a.heads / a.kv_heads, kvh = h / G, row = qi * G + (h - kvh * G);
@@ -644,7 +653,7 @@ __global__ __launch_bounds__(64 * WAVES) void int4_join_kernel(Int4Args a) {
     const int first = cut.worker(u0), last = cut.worker(u0 + start.y - 1);
     if (first == last) return;   // one worker's: stored already
     const int slot = cut.start(first) == u0 ? 0 : 1;
-    const int g = threadIdx.x / T, t = threadIdx.x % T;
+    const int g = threadIdx.x / T, t = threadIdx.x % T, wave = threadIdx.x / 64;
     const int64_t row_at = (int64_t)(kvh % a.head_group) * a.part_rows + row % (16 * NT), worker = 2 * (int64_t)a.head_group * a.part_rows;
     float M = -INFINITY, Ls = 0.0f;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -665,23 +674,31 @@ __global__ __launch_bounds__(64 * WAVES) void int4_join_kernel(Int4Args a) {
                 const int w = w0 + u * PG;
                 const int64_t p = w * worker + (w == first ? slot : 0) * (worker / 2) + row_at;
                 mv[u] = reinterpret_cast<const float2 *>(a.part_ml)[p];
-                ov[u] = reinterpret_cast<const float4 *>(a.part_o)[p * T + t];
+                ov[u] = reinterpret_cast<const float4 *>(a.part_o)[p * (D / 4) + cut_at + t];
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (w0 + u * PG <= last) fold(mv[u].x, mv[u].y, ov[u]);
     }
-    if constexpr (PG > 1) {
-        if (t == 0) ml[g][0] = M, ml[g][1] = Ls;
-        os[g][t] = O;
+#pragma unroll
+    for (int o = T; o < 64; o <<= 1)   // the wave's groups
+        fold(__shfl_xor(M, o, 64), __shfl_xor(Ls, o, 64),
+             make_float4(__shfl_xor(O.x, o, 64), __shfl_xor(O.y, o, 64), __shfl_xor(O.z, o, 64), __shfl_xor(O.w, o, 64)));
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x % 64 < T) {
+            if (t == 0) ml[wave] = make_float2(M, Ls);
+            os[wave][t] = O;
+        }
         __syncthreads();
-        if (g != 0) return;
-        for (int k = 1; k < min(PG, last - first + 1); ++k) fold(ml[k][0], ml[k][1], os[k][t]);
+        if (wave != 0) return;
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) fold(ml[k].x, ml[k].y, os[k][t]);
     }
+    if (g != 0) return;
     const float inv = Ls == 0.0f ? 0.0f : 1.0f / Ls;
     typename Elem<DT>::T v[4] = {Elem<DT>::store(O.x * inv), Elem<DT>::store(O.y * inv), Elem<DT>::store(O.z * inv), Elem<DT>::store(O.w * inv)};
-    __builtin_memcpy(a.out + (((int64_t)b * a.query_len + qi) * a.heads + h) * D + 4 * t, v, 8);
+    __builtin_memcpy(a.out + (((int64_t)b * a.query_len + qi) * a.heads + h) * D + 4 * (cut_at + t), v, 8);
 }
 
 // 16 rows a tile, two tiles a wave where there are more (at 256 dims the second's registers would spill)
@@ -704,11 +721,13 @@ template <int DT, int D, int NG, int NT>
 static void launch_int4_tiles(const Int4Args &a, const Int4Grid &g, bool join, hipStream_t s) {
     int4_walk_kernel<DT, D, NG, NT><<<(unsigned)g.blocks, 256, 0, s>>>(a);
     if (!join) return;
-    // a row cut in many pieces has eight waves to join them, else one
-    const dim3 rows((unsigned)a.heads, (unsigned)a.query_len, (unsigned)a.batch);
+    // a row cut in many pieces has eight waves for every 32 dims to join them, else one for all
     const int64_t walks = (int64_t)a.batch * a.row_tiles * (a.kv_heads / a.head_group);
-    if (walks * 16 < a.workers) int4_join_kernel<DT, D, NT, 8><<<rows, 512, 0, s>>>(a);
-    else int4_join_kernel<DT, D, NT, 1><<<rows, 64, 0, s>>>(a);
+    const dim3 rows((unsigned)a.heads, (unsigned)a.query_len, (unsigned)a.batch);
+    if (walks * 16 < a.workers)
+        int4_join_kernel<DT, D, NT, 8, 8><<<dim3(rows.x * (D / 32), rows.y, rows.z), 512, 0, s>>>(a);
+    else
+        int4_join_kernel<DT, D, NT, 1, D / 4><<<rows, 64, 0, s>>>(a);
 }
 template <int DT, int D, int NG> static void launch_int4(const Int4Args &a, const Int4Grid &g, bool join, hipStream_t s) {
     if (g.tile_rows == 16) launch_int4_tiles<DT, D, NG, 1>(a, g, join, s);
