@@ -10,7 +10,7 @@
 // [row tile][head group][step]) that is cut evenly among the workers of a grid that just fills the
 // chip, whatever the sequences' lengths.  A worker is 1, 2 or 4 neighbouring waves, one to a kv head
 // of the head group, so the heads' short rows (32 to 128 bytes) are read as whole cache lines; each
-// wave keeps a running maximum and sum of its own, and none waits for another.  A sequence that lies
+// wave keeps a running maximum and sum of its own, and reads no other's LDS.  A sequence that lies
 // in one worker is stored at once; the others leave (max, sum, row) partials, two a wave at most,
 // that a second kernel joins.
 //   loads: codes, pairs and page ids go from HBM straight to the wave's LDS, whole rows to an
@@ -25,6 +25,12 @@
 //     (16 tokens of one dim to a lane), P scaled by the token's scale of the group before it is
 //     rounded.  Offsets are summed in f32; the 24 that each code reads too much is taken off by one
 //     more product of the same P with 24.
+// What bounds it, and what it measured (8 kv heads of 128 dims, groups of 128, bf16): 64 tokens over 512
+// to 8192 each, 303 MB of cache, 74.5 us in all, the walk 69.8 (4.3 TB/s, 5.3 with the lines that heads
+// of two blocks fetch twice): the stream, beside 550 vector instructions a step, half of which widen
+// codes; the copies alone took 67 before the heads were kept in step.  Three waves a SIMD (168 registers)
+// where one row tile and one group allow it, else two.  Few steps a wave leave the chain of table, codes,
+// scores and partials: 10.6 us for one token over 777.
 // P is rounded to bf16 once for bf16 outputs (half a step of the output's format, averaged over the
 // tokens); for f16 outputs its rounding error is multiplied too (16 bits in all).
 #include "common.hpp"
