@@ -33,7 +33,7 @@
  *     demand (Matmul: at most 16 MiB, 96 MiB for 256x256 tiles; one-row attention: the paged decode
  *     workspace size, or batch x heads x ceil(seq_k / 256) x (head_dim + 2)
  *     floats; F32 attention: key splits x batch x seq_q (or total_q) x heads x
- *     (head_dim + 2) floats, at most about 100 MB (packed 140 MB); scaled-dot-product attention: see there).
+ *     (head_dim + 2) floats, at most about 100 MB; scaled-dot-product attention: see there).
  *     A growth is stream-ordered on the calling
  *     stream (hipFreeAsync of the old buffer after its last user, then
  *     hipMallocAsync): it never blocks the host.  On a stream that is capturing

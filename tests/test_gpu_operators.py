@@ -222,6 +222,20 @@ def test_append_fp8_bytes_are_the_page_write_s(backend, f, rows, dim):
         assert torch.equal(got, w)
 
 
+@pytest.mark.parametrize("rows", [5, 1100])
+@pytest.mark.parametrize("f,dim,mode", [(BF16, 128, 1), (F32, 64, 0), (F16, 36, 0)])
+def test_append_turns_queries_in_place(backend, rows, f, dim, mode):
+    s = append_state(rows, 4, 2, dim, f, f, 0, 16, False, seed=31)
+    own = append_state(rows, 4, 2, dim, f, f, 0, 16, False, seed=31)
+    cfg = puter_amd.RoPEConfig(Mode=mode)
+    call_append(backend, cfg, s, rows, 4, 2, dim, f, f, 0, 16)
+    own["qout"] = own["dev"][0]
+    call_append(backend, cfg, own, rows, 4, 2, dim, f, f, 0, 16)
+    backend.CheckStatus()
+    for a, b in zip([s["qout"]] + s["pools"], [own["qout"]] + own["pools"]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_append_without_rotation(backend):
     rows, kvh, dim, page = 10, 2, 64, 4
     s = append_state(rows, 3, kvh, dim, BF16, BF16, 0, page, True, seed=8)
@@ -869,6 +883,40 @@ def test_packed_in_a_graph(backend, no_collection):
         refs = packed_refs(q.cpu(), k.cpu(), v.cpu(), lens, lens)
         ref, mag = (torch.cat([r[i] for r in refs]) for i in (0, 1))
         within(out, ref, attention_bound(f, ref, mag, max(r[2] for r in refs), d, 300, p_bits(f)))
+
+
+def test_packed_f32_split_and_in_a_graph(backend, no_collection):
+    """f32's key splits (eager calls on streams of their own, one after another on one scratch) and the
+    unsplit kernel (in a graph): each within the bound, eager calls equal to each other."""
+    h, kv, d, f = 4, 2, 64, F32
+    q, k, v = (randn(70 + i, (700, n, d), f).cuda() for i, n in enumerate((h, kv, kv)))
+    off = torch.tensor([0, 100, 200, 700], dtype=torch.int32).cuda()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [torch.zeros_like(q) for _ in streams]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    replayed = torch.zeros_like(q)
+    with torch.cuda.graph(graph, stream=streams[0]):
+        call_packed(backend, q, k, v, replayed, off, None, h, kv, d, f)
+    for lens in ([100, 100, 500], [1, 698, 1], [0, 0, 700], [129, 128, 300]):
+        off.copy_(torch.tensor(np.concatenate(([0], np.cumsum(lens))), dtype=torch.int32))
+        for t in outs + [replayed]:
+            t.fill_(8.0)
+        torch.cuda.synchronize()
+        for st, o in zip(streams, outs):
+            with torch.cuda.stream(st):
+                call_packed(backend, q, k, v, o, off, None, h, kv, d, f)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        n = sum(lens)
+        refs = packed_refs(q.cpu()[:n], k.cpu()[:n], v.cpu()[:n], lens, lens)
+        ref, mag = (torch.cat([r[i] for r in refs]) for i in (0, 1))
+        bound = attention_bound(f, ref, mag, max(r[2] for r in refs), d, 700, p_bits(f))
+        for o in outs[:1] + [replayed]:
+            within(o[:n], ref, bound, lens)
+            assert (o[n:] == 8.0).all()
+        assert all(torch.equal(o, outs[0]) for o in outs)
 
 
 def test_two_streams_at_once(backend):
