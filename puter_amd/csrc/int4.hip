@@ -26,9 +26,9 @@
 //     rounded.  Offsets are summed in f32; the 24 that each code reads too much is taken off by one
 //     more product of the same P with 24.
 // What bounds it, and what it measured (8 kv heads of 128 dims, groups of 128, bf16): 64 tokens over 512
-// to 8192 each, 303 MB of cache, 74.5 us in all, the walk 69.8 (4.3 TB/s, 5.3 with the lines that heads
-// of two blocks fetch twice): the stream, beside 550 vector instructions a step, half of which widen
-// codes; the copies alone took 67 before the heads were kept in step.  Three waves a SIMD (168 registers)
+// to 8192 each, 303 MB of cache, 73 us in all, the walk 68 (4.5 TB/s): the stream, beside 550 vector instructions a step, half of which widen
+// codes; the copies alone took 67 before the heads were kept in step.  By the clock of its waves: first codes
+// 5 us after the start (contexts, table, codes: one behind the other), then a step at the stream's rate.  Three waves a SIMD (168 registers)
 // where one row tile and one group allow it, else two.  Few steps a wave leave the chain of table, codes,
 // scores and partials: 10.6 us for one token over 777.
 // P is rounded to bf16 once for bf16 outputs (half a step of the output's format, averaged over the
@@ -155,6 +155,12 @@ __device__ __forceinline__ void int4_wait_lds() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+__device__ __forceinline__ void int4_priority(int p) {   // wave-uniform, 0 to 2
+    if (p == 0) __builtin_amdgcn_s_setprio(0);
+    else if (p == 1) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(2);
+}
+
 // Eight codes (nibble k = code k) as 16-bit values 24 + n in the order 0, 4, 1, 5, 2, 6, 3, 7.
 template <bool BF> __device__ __forceinline__ uint4 int4_expand(uint32_t w) {
     if constexpr (BF)
@@ -216,6 +222,13 @@ __global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_
 
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // The oldest of a SIMD's waves goes first, so of the blocks that share a CU the first to come was done
+    // at 41 us and the third at 57 (12 steps each).  Their waves take turns at going first, a step at a
+    // time, the youngest to begin with: 74.5 -> 73 us and 31.2 -> 30.4 (64 sequences, three long ones); waves of
+    // two row tiles lose 5 % by it and keep their age.
+    constexpr int TURNS = NT == 1 ? int4_blocks_per_cu(D, NG, NT) : 1;
+    int turn = blockIdx.x >> 8;
+    if constexpr (TURNS > 1) int4_priority(turn);
     const int G = a.heads / a.kv_heads, R = G * a.query_len;
     const int groups = a.kv_heads / a.head_group;   // head groups
     const int worker = blockIdx.x * (4 / a.head_group) + wave / a.head_group, member = wave % a.head_group;
@@ -368,6 +381,10 @@ __global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_
             prepare_q();
             for (int step = step0; step < step1; ++step) {
                 const bool more = step + 1 < step1;
+                if constexpr (TURNS > 1) {
+                    turn = turn == 0 ? TURNS - 1 : turn - 1;
+                    int4_priority(turn);
+                }
                 if (more) int4_wait_loads<2 * NV + 1>();   // K is there
                 else int4_wait_loads<NV>();
                 const char *const kt = ring + tk, *const vt = ring + tv;
