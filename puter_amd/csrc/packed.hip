@@ -248,7 +248,8 @@ static bool launch_packed_mfma(const PackedMha &m, int dtype, hipStream_t s, int
     // f32: a block's keys are split over blockIdx.y while there are fewer than two blocks a CU, up to
     // about two a CU, in runs of two key tiles or more; each block cuts its own tiles, whose number the
     // host does not know.  2331 rows of five sequences (8 heads of 80, a window of 512): 163 us unsplit,
-    // 74 so, 85 at four splits in place of three, 90 at two; runs of 6 tiles or more lose where
+    // 72 so, 85 at four splits in place of three, 90 at two; runs of one length for all
+    // blocks, from the lengths on the device, 78; runs of 6 tiles or more lose where
     // sequences are short (300 rows, 8 heads of 64: 16 us against 24).  The partials lie in the
     // library's scratch, which cannot grow while a graph is recorded: there the keys stay together.
     int64_t splits = 1;

@@ -1137,6 +1137,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_f32_kernel(Args 
 #pragma unroll
         for (int g = 0; g < 32; ++g) {
             if (g >= T::KG) break;
+            if (PACKED && PAD && 8 * g >= dim) break;   // groups past the head dim add zeros
             const f32x4 kv = *reinterpret_cast<const f32x4 *>(ks + kr + (((2 * g + h) ^ T::kswz(l32)) << 4));
 #pragma unroll
             for (int s4 = 0; s4 < 4; ++s4) sacc = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[s4], qf[g][s4], sacc, 0, 0, 0);
