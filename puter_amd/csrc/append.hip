@@ -177,10 +177,12 @@ struct Int4Group {
 // neighbouring lanes, which find a 4-bit group's range by shuffles.  A wave takes 64 items of one row
 // at a time, so that the row's addresses are scalar, and asks for its next before it works on one.
 //
-// FEW (up to 1024 rows, 1 to 4 a block): latency is all.  Every thread has its first item's loads, its
+// FEW (up to 4096 rows, 1 to 4 a block): latency is all.  Every thread has its first item's loads, its
 // share of the angles and of the later rows' keys (compared with the block's own, one by one) under
 // way at once, and one barrier stands between them and the items.  64 rows of 32 + 8 heads of 128, of
-// a fused QKV row, to bf16 pages: 4.3 us in a graph, most of it one chain of loads and the launch.
+// a fused QKV row, to bf16 pages: 4.2 us in a graph, most of it one chain of loads and the launch (6.4
+// the other way; 1024 rows 8.0 and 11.0, 4096 rows 20 and 24, 8 + 2 heads of 64 to fp8 pages 11.3 and 11.7; at
+// 8192 such rows 22 and 15, as every block reads all later rows' keys).
 //
 // Else the rows that store are settled as the page write settles them (page.hpp), then taken
 // chunk_rows at a time with a table of (cos, sin) for the chunk's positions in LDS.  The rows are
@@ -195,7 +197,7 @@ template <class P> __device__ __forceinline__ P append_pick(bool first, P a, P b
 constexpr int kAppendThreads = 512;
 // blocks a CU, all resident at once: three where an item's 80 registers allow it; two of f32 rows
 constexpr int append_blocks_per_cu(int dt) { return dt == PUTER_F32 ? 2 : 3; }
-constexpr int kFewAppendRows = 1024;
+constexpr int kFewAppendRows = 4096;
 template <int DT, int CACHE, bool FEW>
 __global__ __launch_bounds__(kAppendThreads, FEW ? 4 : 2 * append_blocks_per_cu(DT)) void kv_append_kernel(AppendArgs a) {
 #pragma clang fp contract(off)

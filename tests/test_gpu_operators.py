@@ -103,6 +103,11 @@ APPENDS = [
     (1100, 4, 2, 64, BF16, BF16, 0, 1, 16, True),
     (1500, 2, 2, 128, F16, I4, 32, 1, 64, True),
     (9000, 2, 1, 64, BF16, E4M3, 0, 0, 16, False),
+    (4097, 4, 2, 64, BF16, BF16, 0, 1, 16, True),
+    (4500, 2, 2, 128, F16, I4, 32, 1, 64, True),
+    (6001, 2, 1, 256, BF16, I4, 128, 0, 16, False),
+    (4200, 2, 1, 48, F32, F32, 0, 0, 16, False),
+    (5000, 1, 1, 36, F32, E4M3, 0, 1, 8, True),
 ]
 
 
@@ -199,7 +204,7 @@ def test_append_is_rope_and_page_write(backend, f, mode):
 
 
 @pytest.mark.parametrize("f", [BF16, F16, F32])
-@pytest.mark.parametrize("rows,dim", [(70, 64), (70, 20), (1500, 64)])
+@pytest.mark.parametrize("rows,dim", [(70, 64), (70, 20), (1500, 64), (4500, 64)])
 def test_append_fp8_bytes_are_the_page_write_s(backend, f, rows, dim):
     """Unrotated rows into fp8 pages: byte for byte what KVPageWriteFP8 stores, whatever the scale
     (least, zero, negative, vast, not a number) and the value (ties, infinities, NaN)."""
@@ -222,7 +227,7 @@ def test_append_fp8_bytes_are_the_page_write_s(backend, f, rows, dim):
         assert torch.equal(got, w)
 
 
-@pytest.mark.parametrize("rows", [5, 1100])
+@pytest.mark.parametrize("rows", [5, 1100, 4400])
 @pytest.mark.parametrize("f,dim,mode", [(BF16, 128, 1), (F32, 64, 0), (F16, 36, 0)])
 def test_append_turns_queries_in_place(backend, rows, f, dim, mode):
     s = append_state(rows, 4, 2, dim, f, f, 0, 16, False, seed=31)
@@ -247,7 +252,7 @@ def test_append_without_rotation(backend):
     assert torch.equal(s["qout"], q) and torch.equal(s["pools"][0].cpu()[at], k.cpu()) and torch.equal(s["pools"][1].cpu()[at], v.cpu())
 
 
-@pytest.mark.parametrize("rows", [3, 40, 700, 2500])
+@pytest.mark.parametrize("rows", [3, 40, 700, 2500, 6000])
 @pytest.mark.parametrize("cache", [BF16, E4M3, I4])
 def test_append_last_row_of_a_slot_wins(backend, rows, cache):
     """Several rows of one slot, near and far apart: the last one's K, V and pair stand."""
