@@ -767,8 +767,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefill_kernel(Args a) {
     const int qfirst = q0 + 32 * wave;
     const int qlast = min(qfirst + 31, a.seq_q - 1);
     const int qi = qfirst + l32;
-    // short sequences of a packed batch: a wave without a query only copies
-    const bool idle = PACKED && qfirst >= a.seq_q;
+    // short sequences of a packed batch: a wave without a query only copies (not at 256 dims, where the
+    // branch made 53 to 148 registers spill: 2048 rows, 8 heads 168 us, 104 without; 40 x 30 rows 27 and 20)
+    const bool idle = PACKED && D <= 128 && qfirst >= a.seq_q;
     V8 qf[T::KS];
     {
         const int qload = min(qi, a.seq_q - 1);  // rows past the end compute garbage, never stored

@@ -9,7 +9,8 @@ from test_kernel_resources import kernels  # noqa: F401  (the fixture)
 
 
 @pytest.mark.parametrize("name", ["int4_gather_kernel", "int4_join_kernel", "kv_append_pair_kernel", "packed_f32_combine_kernel",
-                                  r"kv_append_kernelILi\dELi\dELb1E", "kv_append_kernelILi0E"])
+                                  r"kv_append_kernelILi\dELi\dELb1E", "kv_append_kernelILi0E",
+                                  r"prefill_kernelILi\d+ELi\d+ELb\dELb\dENS_10PackedArgs"])
 def test_no_spills(kernels, name):  # noqa: F811
     mine = {n: k[".vgpr_spill_count"] for n, k in kernels.items() if re.search(name, n)}
     assert mine
