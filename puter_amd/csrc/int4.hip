@@ -5,7 +5,7 @@
 // dims.  Query i of a sequence of `context` cached tokens and m queries sees the tokens up to
 // context - m + i.
 //
-// Work: a sequence's cache is walked in steps of 64 tokens, once per kv head and tile of up to 32 of
+// Work: a sequence's cache is walked in steps of 64 tokens, once per kv head and tile of up to 16 of
 // the (query, head) rows that share the kv head.  All steps of the call stand in one line ([sequence]
 // [row tile][head group][step]) that is cut evenly among the workers of a grid that just fills the
 // chip, whatever the sequences' lengths.  A worker is 1, 2 or 4 neighbouring waves, one to a kv head
@@ -29,7 +29,7 @@
 // to 8192 each, 303 MB of cache, 73 us in all, the walk 68 (4.5 TB/s): the stream, beside 550 vector instructions a step, half of which widen
 // codes; the copies alone took 67 before the heads were kept in step.  By the clock of its waves: first codes
 // 5 us after the start (contexts, table, codes: one behind the other), then a step at the stream's rate.  Three waves a SIMD (168 registers)
-// where one row tile and one group allow it, else two.  Few steps a wave leave the chain of table, codes,
+// where one group of 128 dims or heads of 64 allow it, else two (one at 256 dims).  Few steps a wave leave the chain of table, codes,
 // scores and partials: 10.6 us for one token over 777.
 // P is rounded to bf16 once for bf16 outputs (half a step of the output's format, averaged over the
 // tokens); for f16 outputs its rounding error is multiplied too (16 bits in all).
@@ -203,13 +203,18 @@ template <int D> struct Int4Dim {
 };
 
 // Blocks of the walk on a CU, by their registers and LDS.
-constexpr int int4_blocks_per_cu(int dim, int groups, int tiles) { return dim > 128 ? 1 : tiles == 1 && (groups == 1 || dim == 64) ? 3 : 2; }
+constexpr int int4_blocks_per_cu(int dim, int groups) { return dim > 128 ? 1 : groups == 1 || dim == 64 ? 3 : 2; }
 
-// NG: groups of a head; NT: tiles of 16 rows.
-template <int DT, int D, int NG, int NT>
-__global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_kernel(Int4Args a) {
+// NG: groups of a head.
+template <int DT, int D, int NG>
+__global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG)) void int4_walk_kernel(Int4Args a) {
     using L = Int4Dim<D>;
     constexpr bool BF = DT == PUTER_BF16;
+    // Row tiles a wave.  Two share the widening of the codes, but up to 100 of their registers spill and two
+    // waves a SIMD are left: 16 x 5 queries of 4 heads over 3000 tokens of 128 dims 37, 43 and 57 us in
+    // groups of 128, 64 and 32, one at a time 35, 37 and 40; over 6000 tokens 48 and 50, and at 128 rows over
+    // 60000, the most that two gained, 52 and 59.
+    constexpr int NT = 1;
     constexpr int RB = L::RB, KS = D / 32, DC = D / 16, GD = D / NG;
     constexpr int NP = NG >= 4 ? NG / 4 : NG, NV = L::CPR + NP;   // copies of a tile's pairs; of a tile
     constexpr int TILE = 64 * RB + 256 * NG;                      // codes, then pairs
@@ -224,9 +229,8 @@ __global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // The oldest of a SIMD's waves goes first, so of the blocks that share a CU the first to come was done
     // at 41 us and the third at 57 (12 steps each).  Their waves take turns at going first, a step at a
-    // time, the youngest to begin with: 74.5 -> 73 us and 31.2 -> 30.4 (64 sequences, three long ones); waves of
-    // two row tiles lose 5 % by it and keep their age.
-    constexpr int TURNS = NT == 1 ? int4_blocks_per_cu(D, NG, NT) : 1;
+    // time, the youngest to begin with: 74.5 -> 73 us and 31.2 -> 30.4 (64 sequences, three long ones).
+    constexpr int TURNS = int4_blocks_per_cu(D, NG);
     int turn = blockIdx.x >> 8;
     if constexpr (TURNS > 1) int4_priority(turn);
     const int G = a.heads / a.kv_heads, R = G * a.query_len;
@@ -663,7 +667,7 @@ __global__ __launch_bounds__(256, int4_blocks_per_cu(D, NG, NT)) void int4_walk_
 // one order.  T = D / 4 in one wave where there are few pieces a row.  Where there are many (three contexts
 // of 50 to 120 thousand tokens leave 340 a row, 174 KB, for 48 rows), one CU cannot read them fast enough:
 // a block for every 32 dims, with eight waves of eight groups, takes 5.6 us, whole rows by eight waves 9.4.
-template <int DT, int D, int NT, int WAVES, int T>
+template <int DT, int D, int WAVES, int T>
 __global__ __launch_bounds__(64 * WAVES) void int4_join_kernel(Int4Args a) {
     constexpr int CUTS = D / 4 / T, PG = 64 * WAVES / T, U = 8;   // blocks of a row, groups, loads
     __shared__ float2 ml[WAVES];
@@ -672,12 +676,12 @@ __global__ __launch_bounds__(64 * WAVES) void int4_join_kernel(Int4Args a) {
     const int2 start = a.starts[b];
     const Int4Cut cut(a.workers, a.starts[a.batch].x);
     const int G = a.heads / a.kv_heads, kvh = h / G, row = qi * G + (h - kvh * G);
-    const int u0 = start.x + (row / (16 * NT) * (a.kv_heads / a.head_group) + kvh / a.head_group) * start.y;
+    const int u0 = start.x + (row / 16 * (a.kv_heads / a.head_group) + kvh / a.head_group) * start.y;
     const int first = cut.worker(u0), last = cut.worker(u0 + start.y - 1);
     if (first == last) return;   // one worker's: stored already
     const int slot = cut.start(first) == u0 ? 0 : 1;
     const int g = threadIdx.x / T, t = threadIdx.x % T, wave = threadIdx.x / 64;
-    const int64_t row_at = (int64_t)(kvh % a.head_group) * a.part_rows + row % (16 * NT), worker = 2 * (int64_t)a.head_group * a.part_rows;
+    const int64_t row_at = (int64_t)(kvh % a.head_group) * a.part_rows + row % 16, worker = 2 * (int64_t)a.head_group * a.part_rows;
     float M = -INFINITY, Ls = 0.0f;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto fold = [&](float pm, float pls, float4 po) __attribute__((always_inline)) {
@@ -724,37 +728,29 @@ __global__ __launch_bounds__(64 * WAVES) void int4_join_kernel(Int4Args a) {
     __builtin_memcpy(a.out + (((int64_t)b * a.query_len + qi) * a.heads + h) * D + 4 * (cut_at + t), v, 8);
 }
 
-// 16 rows a tile, two tiles a wave where there are more (at 256 dims the second's registers would spill)
-static int64_t int4_tile_rows(int64_t rows, int64_t dim) { return rows <= 16 || dim > 128 ? 16 : 32; }
 // The grid: blocks that fill the chip (by their LDS and registers), fewer where there are fewer steps.
 struct Int4Grid {
-    int64_t head_group, row_tiles, tile_rows, blocks, part_rows, steps;
+    int64_t head_group, row_tiles, blocks, part_rows, steps;
     Int4Grid(int64_t batch, int64_t query_len, int64_t heads, int64_t kv_heads, int64_t dim, int64_t group, int64_t max_context) {
         const int64_t rows = heads / kv_heads * query_len;
         head_group = kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
-        tile_rows = int4_tile_rows(rows, dim);
-        row_tiles = (rows + tile_rows - 1) / tile_rows;
-        part_rows = std::min(rows, tile_rows);
+        row_tiles = (rows + 15) / 16;
+        part_rows = std::min<int64_t>(rows, 16);
         steps = batch * row_tiles * (kv_heads / head_group) * ((max_context + 63) / 64);
-        blocks = std::min<int64_t>(256 * int4_blocks_per_cu((int)dim, (int)(dim / group), (int)tile_rows / 16), (steps * head_group + 3) / 4);
+        blocks = std::min<int64_t>(256 * int4_blocks_per_cu((int)dim, (int)(dim / group)), (steps * head_group + 3) / 4);
     }
 };
 
-template <int DT, int D, int NG, int NT>
-static void launch_int4_tiles(const Int4Args &a, const Int4Grid &g, bool join, hipStream_t s) {
-    int4_walk_kernel<DT, D, NG, NT><<<(unsigned)g.blocks, 256, 0, s>>>(a);
+template <int DT, int D, int NG> static void launch_int4(const Int4Args &a, const Int4Grid &g, bool join, hipStream_t s) {
+    int4_walk_kernel<DT, D, NG><<<(unsigned)g.blocks, 256, 0, s>>>(a);
     if (!join) return;
     // a row cut in many pieces has eight waves for every 32 dims to join them, else one for all
     const int64_t walks = (int64_t)a.batch * a.row_tiles * (a.kv_heads / a.head_group);
     const dim3 rows((unsigned)a.heads, (unsigned)a.query_len, (unsigned)a.batch);
     if (walks * 16 < a.workers)
-        int4_join_kernel<DT, D, NT, 8, 8><<<dim3(rows.x * (D / 32), rows.y, rows.z), 512, 0, s>>>(a);
+        int4_join_kernel<DT, D, 8, 8><<<dim3(rows.x * (D / 32), rows.y, rows.z), 512, 0, s>>>(a);
     else
-        int4_join_kernel<DT, D, NT, 1, D / 4><<<rows, 64, 0, s>>>(a);
-}
-template <int DT, int D, int NG> static void launch_int4(const Int4Args &a, const Int4Grid &g, bool join, hipStream_t s) {
-    if (g.tile_rows == 16) launch_int4_tiles<DT, D, NG, 1>(a, g, join, s);
-    else launch_int4_tiles<DT, D, NG, D <= 128 ? 2 : 1>(a, g, join, s);
+        int4_join_kernel<DT, D, 1, D / 4><<<rows, 64, 0, s>>>(a);
 }
 template <int DT> static void launch_int4_dim(const Int4Args &a, int dim, int group, const Int4Grid &g, bool join, hipStream_t s) {
     switch (1000 * dim + group) {

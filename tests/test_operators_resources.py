@@ -20,14 +20,14 @@ def test_no_spills(kernels, name):  # noqa: F811
 def test_blocks_of_the_4_bit_walk_fit_a_cu(kernels):  # noqa: F811
     seen = 0
     for n, k in kernels.items():
-        m = re.search(r"int4_walk_kernelILi\dELi(\d+)ELi(\d)ELi(\d)E", n)
+        m = re.search(r"int4_walk_kernelILi\dELi(\d+)ELi(\d)E", n)
         if not m:
             continue
         seen += 1
-        dim, groups, tiles = map(int, m.groups())
-        blocks = 1 if dim > 128 else 3 if tiles == 1 and (groups == 1 or dim == 64) else 2
+        dim, groups = map(int, m.groups())
+        blocks = 1 if dim > 128 else 3 if groups == 1 or dim == 64 else 2
         lds = -(-k[".group_segment_fixed_size"] // 1280) * 1280   # what a block is given
         assert blocks * lds <= 160 * 1024, n
         # four waves a block, one on each SIMD of 512 registers a lane
         assert blocks * (-(-k[".vgpr_count"] // 8) * 8) <= 512, n
-    assert seen == 26
+    assert seen == 16
